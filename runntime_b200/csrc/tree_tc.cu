@@ -13,18 +13,20 @@
 // a part's end or beginning, the other goes on.  More rows are taken two tiles at a time by the two warpgroups of one
 // stream, which share every K and V tile: read by a block each, they met the limit of the L2.  (One
 // warpgroup after another on the tiles of one part, sharing the rows' reference points, the scheme of the prefill
-// kernel, stopped at every part's end: 32 x 8190 rows, 25 tokens 200 us, now 161; 65001 rows, 64 tokens 102, now 92.)
+// kernel, stopped at every part's end: 32 x 8190 rows, 25 tokens 200 us for 161; 65001 rows, 64 tokens 102 for 92, both with
+// probabilities of one half.)
 //
-// What it takes with 32 heads on 8 of 128: 32 sequences of 8190 rows, 25 tokens 161 us, 5.2 TB/s (the caches' bytes at
-// the copy rate: 128); 16 of 4096 at most, 16 tokens 53 us, 3.9 TB/s, of which some 9 pass before the first product and 6 in
-// the joining launch; one of 65001, 64 tokens 92 us, 740 TFLOP/s: of some 2100 cycles a tile a warpgroup works 1300 and waits
-// 650 for its next scores, whose product follows that of the probabilities whose place they take.  (A quarter of the
-// exponentials on the FMA pipe: 96 us; three eighths: 100.)  The smallest, 8 heads of 52, 190 rows and 7 tokens: 12 us, all of
-// it latency.
+// What it takes with 32 heads on 8 of 128: 32 sequences of 8190 rows, 25 tokens 187 us, 4.5 TB/s (the caches' bytes at
+// the copy rate: 128); 16 of 4096 at most, 16 tokens 55.5 us, 3.7 TB/s, of which some 9 pass before the first product and 6 in
+// the joining launch; one of 65001, 64 tokens 111 us, 614 TFLOP/s counting each product once: a chain of scores, softmax and the
+// product of the probabilities, whose place the next scores take.  (Probabilities of one half, 11 bits: 162, 53 and 92 us.)
+// The smallest, 8 heads of 52, 190 rows and 7 tokens: 12 us, all of it latency.
 //
 // A producer warp for each stream fills rings of K and V tiles by TMA that run on across the parts' ends.  Scores have
-// two buffers of 64 columns; the probabilities take their scores' place.  A row's reference point moves only when
-// its maximum has grown by more than 2^13, and O is rescaled then.
+// two buffers of 64 columns; the probabilities take their scores' place, each as two halves, its upper eleven bits and
+// the rest, that are multiplied by the same values: one half alone made results half again as far off as
+// their own rounding to f16 does.  A row's reference point moves only when its maximum has grown by more than seven
+// binary orders, and O is rescaled then.
 //
 // What a row does not see has no part in its result, whatever it holds: values past the length, and values
 // that are not finite in tiles that some rows see in part, are cleared in shared memory, and a row whose result
@@ -46,6 +48,10 @@ constexpr int kThreads = 384;
 constexpr int BK = 64;                               // keys of a tile
 static_assert(BK == RT_MAX_NODES, "the nodes' own keys are one tile");
 constexpr float kLn2 = 0.6931471805599453f;
+// A row's reference point is set kLift binary orders below its maximum and moves when the maximum is kTop above it: a
+// probability, 2^(s - reference) in f32, is at most 2^15, and what two halves leave of it is 2^-22 of it or
+// 2^-25, which is 2^-33 of the row's largest.  (kLift 10, 6 and 2: 65001 rows and 64 tokens 112, 110 and 108 us, with 8 111.)
+constexpr float kLift = 8.f, kTop = 15.f;
 
 template <int HD>
 struct Cfg {
@@ -318,7 +324,7 @@ __device__ __forceinline__ TreeRow row_of_part(const TreeParams& p, const Part& 
   seen = kNegSeed;
   if (node < part.nodes) {
     if (part.t0 == 0 || p.wl != RT_WINDOW_INF) row = tree_row(p, part.b, node, part.rows, part.nodes);
-    if (p.sinks && part.t0 == 0) seen = fmaxf(p.sinks[head], kNegSeed);   // (in the log2 domain)
+    if (p.sinks && part.t0 == 0) seen = fmaxf(p.sinks[head] - kLift, kNegSeed);   // (in the log2 domain)
   }
   return row;
 }
@@ -682,14 +688,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
           if (elect_one()) {
             const uint32_t bLo = (((sV + slot * C::SLOT_BYTES) & 0x3ffffu) >> 4) | kLboV;
             const uint32_t pCol = sCol + (j & 1) * BK;
+            auto product = [&](int kk) {   // 16 keys, the probabilities' upper and lower halves
+              const uint64_t v = desc(bLo + kk * (2048 >> 4));
+              mma_f16_ts(oCol, pCol + kk * 8, v, idescO, (i > 0 || kk > 0) ? 1u : 0u);
+              mma_f16_ts(oCol, pCol + BK / 2 + kk * 8, v, idescO, 1u);
+            };
             if (steps == BK / 16) {
 #pragma unroll
-              for (int kk = 0; kk < BK / 16; kk++)
-                mma_f16_ts(oCol, pCol + kk * 8, desc(bLo + kk * (2048 >> 4)), idescO, (i > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < BK / 16; kk++) product(kk);
             } else {
 #pragma unroll 1
-              for (int kk = 0; kk < steps; kk++)
-                mma_f16_ts(oCol, pCol + kk * 8, desc(bLo + kk * (2048 >> 4)), idescO, (i > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < steps; kk++) product(kk);
             }
             tc_commit(bar(sh.vEmpty[slot]));
             tc_commit(bar(sh.pvDone[g][j & 1]));
@@ -731,7 +740,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
       }
       float seen;        // the row's reference point (log2 domain)
       const TreeRow row = row_of_part(p, part, node, head, seen);
-      float l = seen != kNegSeed ? 1.f : 0.f;      // the row's sink
+      float l = seen != kNegSeed ? exp2f(kLift) : 0.f;      // the row's sink
       unsigned long long* const spoilt = &sh.spoilt[s][live % kFlags];
       int* const spoiltRow = &sh.spoiltRow[s][live % kFlags];
       if (rowInTile == 0 && (g == 0 || plan.solo))
@@ -773,12 +782,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
 #pragma unroll
             for (int u = 0; u < 4; u++) mx4[u] = max3(mx4[u], __uint_as_float(sv[c + 2 * u]), __uint_as_float(sv[c + 2 * u + 1]));
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * kLog2e;
-          const bool grow = mx > seen + kRescaleThreshold;
+          const bool grow = mx > seen + kTop;
           if (__any_sync(0xffffffffu, grow)) {
             // A row whose reference point is still the seed has met no key: its accumulator row is zero.
             const bool pass = i > 0 && __any_sync(0xffffffffu, grow && seen != kNegSeed);
             // (a row moves by itself: rows without a node, whose scores are whatever was there, move no other)
-            const float mnew = grow || i == 0 || seen == kNegSeed ? fmaxf(seen, mx) : seen;
+            const float mnew = grow || i == 0 || seen == kNegSeed ? fmaxf(seen, mx - kLift) : seen;
             const float f = fast_exp2(seen - mnew);
             if (pass) {
               // (S(j) is there: P V(j-2) is done, and the open phase of the other barrier is P V(j-1)'s)
@@ -801,7 +810,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
           }
           const float2 scale2 = make_float2(kLog2e, kLog2e), shift2 = make_float2(-seen, -seen);
           float2 sum2[4];
-          uint32_t pk[32];
+          uint32_t hi[32], lo[32];
 #pragma unroll
           for (int u = 0; u < 4; u++) sum2[u] = make_float2(0.f, 0.f);
 #pragma unroll
@@ -809,12 +818,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
             const float2 x = fma2(make_float2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, shift2);
             const float2 pe = make_float2(fast_exp2(x.x), fast_exp2(x.y));
             sum2[(c >> 1) & 3] = add2(sum2[(c >> 1) & 3], pe);
-            const __half2 hp = __floats2half2_rn(pe.x, pe.y);
-            pk[c / 2] = *reinterpret_cast<const uint32_t*>(&hp);
+            // the upper eleven bits as they are, and what is left of it
+            const float2 up = make_float2(__uint_as_float(__float_as_uint(pe.x) & 0xffffe000u), __uint_as_float(__float_as_uint(pe.y) & 0xffffe000u));
+            const float2 rest = fma2(up, make_float2(-1.f, -1.f), pe);
+            const __half2 hp = __floats2half2_rn(up.x, up.y), lp = __floats2half2_rn(rest.x, rest.y);
+            hi[c / 2] = *reinterpret_cast<const uint32_t*>(&hp);
+            lo[c / 2] = *reinterpret_cast<const uint32_t*>(&lp);
           }
           const float2 s01 = add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3]));
           l += s01.x + s01.y;
-          tmem_st32(sBuf, pk);   // P in its scores' place
+          tmem_st32(sBuf, hi);   // P in its scores' place
+          tmem_st32(sBuf + BK / 2, lo);
           tmem_wait_st();
         }
         tc_fence_before_sync();
