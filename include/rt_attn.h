@@ -79,7 +79,9 @@ RT_API int rt_ctx_set_stream(rt_ctx* ctx, void* cuda_stream, int external);
 #define RT_OPT_PREFILL_TC 1
 /* RT_OPT_WAIT_POLLS (default 1 << 20, about a second): how often the merge of a
  * cross-GPU decode step polls for the other ranks' rows before it gives up, writes
- * zeros and makes rt_sync return RT_EXECUTION_FAILED. */
+ * zeros and makes rt_sync return RT_EXECUTION_FAILED.  The same limit (at most 1 << 24)
+ * holds for rt_attn_tree's waits for a free place among its tiles on the tensor cores; it leaves
+ * out unfinished where it gives up. */
 #define RT_OPT_WAIT_POLLS 2
 RT_API int rt_ctx_set_option(rt_ctx* ctx, int option, int value);
 /* Message of the last failure on this context (or, with ctx == NULL, of the

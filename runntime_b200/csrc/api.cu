@@ -31,7 +31,7 @@ struct rt_ctx {
   int* work;         // device: the persistent prefill kernel's queue (units drawn, CTAs finished)
   int64_t launches;
   int useTc;
-  int waitPolls;   // polls of the cross-GPU merge's wait before it gives up
+  int waitPolls;   // polls of a wait of the cross-GPU merge or of tree attention before it gives up
   std::string err;
 };
 
@@ -948,6 +948,7 @@ static rt::TreeParams tree_params(rt_ctx* ctx, const rt_tree_args* a) {
   p.kvLen = a->kvLens && a->kvLen == 0 ? a->cacheRows : a->kvLen;   // (lengths alone: plan for full caches)
   p.qHeads = a->qHeads, p.kvHeads = a->kvHeads, p.hd = a->headDim;
   p.wl = a->windowLeft, p.sharedMasks = a->sharedMasks, p.splits = a->splits;
+  p.polls = (uint32_t)std::min(ctx->waitPolls, 1 << 24);
   return p;
 }
 

@@ -35,6 +35,7 @@ struct TreeParams {
   int* status;
   int64_t cacheSeqStride, qStride, kNewStride, vNewStride;   // elements
   int32_t batch, nodes, cacheRows, kvLen, qHeads, kvHeads, hd, wl, sharedMasks, splits;
+  uint32_t polls;       // for a free place in a ring of tiles before the kernel gives up
 };
 
 #ifdef __CUDACC__

@@ -83,6 +83,9 @@ struct Shared {
   unsigned long long spoilt[2][kFlags];   // nodes whose values are not all finite, by the part's number
   int spoiltRow[2][kFlags];               // and the last such cache row among tiles that some rows see in part, or -1
   Part part[2][2];
+  // Tiles of keys and of values that a stream has asked for, Qs of a warpgroup: what may be on its way when a block gives up.
+  int asked[2][2], askedQ[2];
+  uint64_t over[2];                                   // then: all products of a warpgroup are done
   uint32_t tmem;
   int abort;
 };
@@ -223,10 +226,31 @@ __device__ __forceinline__ void load_tile(const CUtensorMap* map, const Plan& pl
   for (int c = 0; c < HD / 64; c++) tma_load_4d(dst + c * chunkBytes, map, x0 + c * 64, h, y, walk.b, bar);
 }
 
-// After a failed wait: no block leaves while a copy into its shared memory is on its way (waits with a limit, too).
-__device__ __forceinline__ void drain(uint64_t* full, int slots, int issued) {
+// After a failed wait, by all warps of the block: it does not end, and its shared memory is nobody else's, while copies into it
+// and products that read it may be on their way, also those of a role that had come to its end before.  (Waits with a
+// limit, too.)
+__device__ __noinline__ void wait_for_what_is_asked(Shared& sh, int nK, int nV) {
   volatile int never = 0;
-  for (int q = max(issued - slots, 0); q < issued; q++) mbar_poll_warp(smem_u32(&full[q % slots]), (q / slots) & 1, &never);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto all = [&](uint64_t* full, int slots, int asked) {
+    for (int q = max(asked - slots, 0); q < asked; q++) mbar_poll_warp(smem_u32(&full[q % slots]), (q / slots) & 1, &never);
+  };
+  if (warp == 8 || warp == 11) {
+    const int s = warp == 11;
+    all(sh.kFull + s * nK, nK, sh.asked[s][0]);
+    all(sh.vFull + s * nV, nV, sh.asked[s][1]);
+  } else if (warp == 9 || warp == 10) {
+    const int g = warp - 9;
+    all(&sh.qFull[g], 1, sh.askedQ[g]);
+    if (lane == 0) {
+      mbar_init(smem_u32(&sh.over[g]), 1);
+      fence_barrier_init();
+    }
+    __syncwarp();
+    if (elect_one()) tc_commit(smem_u32(&sh.over[g]));
+    __syncwarp();
+    mbar_poll_warp(smem_u32(&sh.over[g]), 0, &never);
+  }
 }
 
 // One row over a part's tiles, key by key, by one warp: the result's columns (lane,
@@ -556,10 +580,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
   if (warp == 8 || warp == 11) {
     // ------------------------------ keys and values of a stream ------------------------------
     const int s = warp == 8 ? 0 : 1;
+    int count[2] = {0, 0};
     if (ok && (s == 0 || plan.solo) && active(s)) {
       // The next tile of keys and the next one of values, each fetched when its slot is free.
       Walk walks[2] = {walk, walk};
-      int at[2], count[2] = {0, 0};
+      int at[2];
       bool more[2];
       auto forward = [&](Walk& w, int& t, bool& m) {
         while (m && t == w.t1) {
@@ -597,29 +622,27 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
           idle = 0;
           continue;
         }
-        // (the limit is that of the other waits, a second or two)
-        if (++idle > (1u << 24) || (idle % 32 == 0 && *abortFlag)) {
+        // (the limit is that of the other waits, a second or two, by default; a limit of one poll does not wait at all)
+        if (idle++ / 16 + 1 >= p.polls || (idle % 32 == 0 && *abortFlag)) {
           *abortFlag = 1;
           break;
         }
         __nanosleep(64);
         __syncwarp();
       }
-      if (*abortFlag) {   // no block leaves while a copy into its shared memory is on its way
-        drain(sh.kFull + s * nK, nK, count[0]);
-        drain(sh.vFull + s * nV, nV, count[1]);
-      }
     }
+    if (lane == 0) sh.asked[s][0] = count[0], sh.asked[s][1] = count[1];
   } else if (warp == 9 || warp == 10) {
     // ------------------------------ MMA issuer of a warpgroup, and its parts' beginnings ------------------------------
     const int g = warp - 9, s = stream_of(g), mTile = tile_of(g);
+    int qParts = 0;   // parts with a Q
     if (ok && active(g)) {
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // SBO, version, SW128
       constexpr uint32_t kLboK = (16u >> 4) << 16, kLboV = ((uint32_t)(BK * 128) >> 4) << 16;   // V: next 64 columns
       auto desc = [](uint32_t lo32) { return ((uint64_t)kDescHi << 32) | lo32; };
       const uint32_t myQ = sQ + g * C::Q_BYTES, aLo = ((myQ & 0x3ffffu) >> 4) | kLboK;
       const uint32_t sCol = tmem + g * C::WG_COLS + C::S_COL, oCol = tmem + g * C::WG_COLS + C::O_COL;
-      int j = 0, index = 0, seen = 0, qParts = 0;   // tiles, parts, tiles looked through, parts with a Q
+      int j = 0, index = 0, seen = 0;   // tiles, parts, tiles looked through
       for (; ok && walk.next(p, plan); walk.advance(), index++) {
         const int shift = shift_of(walk.kvh), n = walk.t1 - walk.t0;
         // (the part before last is over; the last one's scores are all there, so Q is read no more)
@@ -706,10 +729,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
           __syncwarp();
         }
       }
-      if (!ok && qParts > 0) {   // (a Q on its way, as with the rings)
-        volatile int never = 0;
-        mbar_poll_warp(bar(sh.qFull[g]), (qParts - 1) & 1, &never);
-      }
       if (ok && index >= 2) ok = wait(sh.partDone[g][index & 1], index / 2 - 1);
       if (ok && lane == 0) {
         sh.part[g][index & 1].t0 = -1;   // no more
@@ -717,6 +736,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
       }
       if (!ok) *abortFlag = 1;
     }
+    if (lane == 0) sh.askedQ[g] = qParts;
   } else {
     // ------------------------------ softmax and results of a warpgroup ------------------------------
     const int g = warp >> 2, s = stream_of(g), mTile = tile_of(g), rowInTile = tid & 127;
@@ -865,7 +885,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
   // Common exit: every role arrives here, then the allocating warp frees tensor memory.
   tc_fence_before_sync();
   __syncthreads();
-  if (tid == 0 && *abortFlag) atomicOr(p.status, kStatusWaitTimeout);
+  if (*abortFlag) {
+    wait_for_what_is_asked(sh, nK, nV);
+    if (tid == 0) atomicOr(p.status, kStatusWaitTimeout);
+    __syncthreads();
+  }
   if (warp == 9) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, C::TMEM_COLS);
