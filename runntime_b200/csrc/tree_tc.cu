@@ -102,7 +102,7 @@ struct Plan {
   float* acc;               // [groups][2][mTiles][HD/4][128][4]
   float* ml;                // [groups][2][mTiles][128][2]
   int2* joins;              // [batch * kvHeads]: twice the run of its first part, plus that part's place (-1: it is the only
-                            // one); the run of its last part
+                            // one); the run of its last part.  Unwritten where the launch that writes it has given up
 };
 
 // Tiles of a sequence: one of the nodes' own keys, then the cache's from `first` on.
@@ -921,6 +921,8 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const TreeParams p, 
     if (join.x < 0) return;
     // The runs after the first begin inside the head, so that it is their first part.
     const int g0 = join.x >> 1, g1 = join.y;
+    // (a first launch that gave up has left the table unwritten, and in the scratch may be anything)
+    if (g1 < g0 || g1 >= plan.groups) return;
     auto place = [&](int g) { return ((int64_t)g * 2 + (g == g0 ? join.x & 1 : 0)) * plan.mTiles + mTile; };
     float m = kNegSeed;
 #pragma unroll 8

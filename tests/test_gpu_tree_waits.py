@@ -40,3 +40,24 @@ def test_tree_gives_up(on_torch, polls, shape, nodes):
         gives_up(on_torch)             # (of the call before)
         assert t.torch.equal(got, want)
     on_torch.sync()
+
+
+@pytest.mark.parametrize("shape,nodes", CASES)
+def test_tree_gives_up_before_the_joining_launch(on_torch, polls, shape, nodes):
+    """The launch that joins the parts comes after one that has given up, and finds another call's floats where the
+    places of the parts would be: it joins nothing outside of its scratch."""
+    other = Tree("f32", 8, 2, 64, 64, [2000] * 8, seed=9)
+    t = Tree("f16", *shape, nodes, [20000, 9000, 15000], seed=nodes)    # (more tiles to a run than a ring has places)
+    want = t.call(on_torch, splits=5).clone()
+    on_torch.sync()
+    t.check(want)
+    for _ in range(5):
+        other.call(on_torch, splits=64)     # partial results all over the scratch
+        polls(1)
+        t.call(on_torch, splits=5)
+        polls(DEFAULT)
+        t.out.fill_(7.0)
+        got = t.call(on_torch, splits=5)
+        gives_up(on_torch)
+        assert t.torch.equal(got, want)
+    on_torch.sync()
