@@ -30,7 +30,7 @@
 //
 // What a row does not see has no part in its result, whatever it holds: values past the length, and values
 // that are not finite in tiles that some rows see in part, are cleared in shared memory, and a row whose result
-// is not finite, or that sees a cleared value, is computed again key by key.
+// is not finite, or that sees a cleared value, is computed again key by key at the block's end.
 #include <algorithm>
 #include <climits>
 
@@ -86,6 +86,7 @@ struct Shared {
   // Tiles of keys and of values that a stream has asked for, Qs of a warpgroup: what may be on its way when a block gives up.
   int asked[2][2], askedQ[2];
   uint64_t over[2];                                   // then: all products of a warpgroup are done
+  int marked[2];                                      // whether rows of a warpgroup are to be computed again
   uint32_t tmem;
   int abort;
 };
@@ -253,40 +254,73 @@ __device__ __noinline__ void wait_for_what_is_asked(Shared& sh, int nK, int nV) 
   }
 }
 
-// One row over a part's tiles, key by key, by one warp: the result's columns (lane,
-// lane + 32, ...), the maximum and the sum.
+// One row over a part's tiles by one warp, a key to a lane for the scores: the result's columns (lane, lane + 32, ...), the
+// maximum and the sum.
 __device__ __forceinline__ void exact_tree_row(const TreeParams& p, const Part& s, int node, int head, const TreeRow& row,
                                                float (&acc)[4], float& m, float& l) {
-  const int lane = threadIdx.x & 31, hd = p.hd, b = s.b, kvh = s.kvh, t0 = s.t0, t1 = s.t1;
-  const __half* q = static_cast<const __half*>(p.q) + ((int64_t)b * p.nodes + node) * p.qStride + (int64_t)head * hd;
-  m = p.sinks && t0 == 0 ? fmaxf(p.sinks[head] * kLn2, kNegSeed) : kNegSeed;
+  const int lane = threadIdx.x & 31, hd = p.hd;
+  const __half* q = static_cast<const __half*>(p.q) + ((int64_t)s.b * p.nodes + node) * p.qStride + (int64_t)head * hd;
+  // (rows of keys begin on 16-byte boundaries, heads and queries where hd and q's stride let them)
+  const bool wide = hd % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  m = p.sinks && s.t0 == 0 ? fmaxf(p.sinks[head] * kLn2, kNegSeed) : kNegSeed;
   l = m > kNegSeed ? 1.f : 0.f;
 #pragma unroll
   for (int c = 0; c < 4; c++) acc[c] = 0.f;
-  for (int t = t0; t < t1; t++) {
+  for (int t = s.t0; t < s.t1; t++) {
     const bool own = t == 0;
     const int key0 = own ? 0 : (s.first + t - 1) * BK, end = own ? s.nodes : min(s.rows, key0 + BK);
-    for (int j = key0; j < end; j++) {
-      if (own ? !(row.nodes >> j & 1) : j < row.lo) continue;
-      const __half *k, *v;
-      if (own) {
-        k = static_cast<const __half*>(p.kNew) + ((int64_t)b * p.nodes + j) * p.kNewStride;
-        v = static_cast<const __half*>(p.vNew) + ((int64_t)b * p.nodes + j) * p.vNewStride;
-      } else {
-        const int64_t at = b * p.cacheSeqStride + (int64_t)j * p.kvHeads * hd;
-        k = static_cast<const __half*>(p.kCache) + at;
-        v = static_cast<const __half*>(p.vCache) + at;
-      }
+    const int64_t stride = own ? p.kNewStride : (int64_t)p.kvHeads * hd, vStride = own ? p.vNewStride : stride;
+    const int64_t column = (int64_t)s.kvh * hd;
+    const __half* k = own ? static_cast<const __half*>(p.kNew) + (int64_t)s.b * p.nodes * p.kNewStride
+                          : static_cast<const __half*>(p.kCache) + s.b * p.cacheSeqStride;
+    const __half* v = own ? static_cast<const __half*>(p.vNew) + (int64_t)s.b * p.nodes * p.vNewStride
+                          : static_cast<const __half*>(p.vCache) + s.b * p.cacheSeqStride;
+    for (int j0 = key0; j0 < end; j0 += 32) {
+      const int j = j0 + lane;
+      const bool sees = j < end && (own ? (row.nodes >> j & 1) != 0 : j >= row.lo);
+      if (!__any_sync(0xffffffffu, sees)) continue;
       float x = 0.f;
-      for (int c = lane; c < hd; c += 32) x = fmaf(__half2float(q[c]), __half2float(k[(int64_t)kvh * hd + c]), x);
-      x = warp_sum(x);
-      const float mNew = fmaxf(m, x), f = fast_exp2((m - mNew) * kLog2e), w = fast_exp2((x - mNew) * kLog2e);
-      l = l * f + w;
+      if (sees) {
+        const __half* kj = k + j * stride + column;
+        if (wide) {
+#pragma unroll 8
+          for (int c = 0; c < hd; c += 8) {
+            const uint4 a = *reinterpret_cast<const uint4*>(q + c), b = *reinterpret_cast<const uint4*>(kj + c);
+            const __half2 *a2 = reinterpret_cast<const __half2*>(&a), *b2 = reinterpret_cast<const __half2*>(&b);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float2 u = __half22float2(a2[e]), w = __half22float2(b2[e]);
+              x = fmaf(u.y, w.y, fmaf(u.x, w.x, x));
+            }
+          }
+        } else {
+#pragma unroll 8
+          for (int c = 0; c < hd; c++) x = fmaf(__half2float(q[c]), __half2float(kj[c]), x);
+        }
+      }
+      const float mNew = fmaxf(m, warp_max(sees ? x : -INFINITY)), f = fast_exp2((m - mNew) * kLog2e);
+      const float mine = sees ? fast_exp2((x - mNew) * kLog2e) : 0.f;
+      l = l * f + warp_sum(mine);
       m = mNew;
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        acc[c] *= f;
-        if (w != 0.f && lane + 32 * c < hd) acc[c] = fmaf(w, __half2float(v[(int64_t)kvh * hd + lane + 32 * c]), acc[c]);
+      for (int c = 0; c < 4; c++) acc[c] *= f;
+      // (eight keys' values on their way at a time; those past the last key are the last key's, with no weight)
+      const int keys = min(end - j0, 32);
+#pragma unroll 1
+      for (int i0 = 0; i0 < keys; i0 += 8) {
+        __half x[8][4];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const __half* vi = v + (j0 + min(i0 + i, keys - 1)) * vStride + column;
+#pragma unroll
+          for (int c = 0; c < 4; c++) x[i][c] = lane + 32 * c < hd ? vi[lane + 32 * c] : __half(0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float w = __shfl_sync(0xffffffffu, mine, i0 + i);
+#pragma unroll
+          for (int c = 0; c < 4; c++) acc[c] = w != 0.f ? fmaf(w, __half2float(x[i][c]), acc[c]) : acc[c];
+        }
       }
     }
   }
@@ -420,11 +454,17 @@ __device__ __noinline__ void no_nodes(const TreeParams& p, const Part& part, int
   for (int c = 0; c < hd; c++) out[c] = __float2half_rn(0.f);
 }
 
-// The results of a part's rows: to `out` where the part is a whole (sequence, kv head), else as (m, l, acc).  Returns
-// the warp's rows that are to be computed again, a bit each: the `odd` ones and those that are not finite.
+// What a row that is to be computed again has in the place of its first column, or of its sum: NaNs that no arithmetic makes.
+constexpr unsigned short kAgain = 0x7e01;
+constexpr uint32_t kAgainSum = 0x7fc00001u;
+
+// The results of a part's rows: to `out` where the part is a whole (sequence, kv head), else as (m, l, acc).  Returns whether
+// the row has been marked: the `odd` ones and those that are not finite.  Where a row's scores are all its own (settled: no
+// neighbour's columns were multiplied by zeros) a sum that is NaN comes from a score that it sees, and
+// the row is NaN as it should be.
 template <int HD, bool PADDED>
-__device__ __forceinline__ uint32_t store_rows(const TreeParams& p, const Part& part, int node, int head, bool here, int shift,
-                                               uint32_t oCol, float m, float l, bool odd, float* acc, float* ml) {
+__device__ __forceinline__ bool store_rows(const TreeParams& p, const Part& part, int node, int head, bool here, int shift,
+                                           uint32_t oCol, float m, float l, bool odd, bool settled, float* acc, float* ml) {
   const int rowInTile = threadIdx.x & 127, hd = PADDED ? p.hd : HD;
   const bool final = part.t0 == 0 && part.t1 == part.tiles;
   const bool valid = node < part.nodes;
@@ -469,31 +509,47 @@ __device__ __forceinline__ uint32_t store_rows(const TreeParams& p, const Part& 
           out[c + x - shift] = __ushort_as_half((unsigned short)(x & 1 ? o[x / 2] >> 16 : o[x / 2]));
     }
   }
-  if (!final && here) *reinterpret_cast<float2*>(ml + 2 * rowInTile) = make_float2(m * kLn2, valid ? l : 0.f);
-  return __ballot_sync(0xffffffffu, (odd || check != 0.f) && here && valid);
+  const bool again = (odd || check != 0.f) && here && valid && !(settled && l != l);
+  if (!final && here)
+    *reinterpret_cast<float2*>(ml + 2 * rowInTile) = make_float2(m * kLn2, again ? __uint_as_float(kAgainSum) : valid ? l : 0.f);
+  if (final && again) *reinterpret_cast<unsigned short*>(out) = kAgain;
+  return again;
 }
 
-// The marked rows of a warp, key by key.
-__device__ __noinline__ void redo_rows(const TreeParams& p, const Part& part, int mTile, int shift, uint32_t redo, float* acc, float* ml) {
-  const int lane = threadIdx.x & 31, heads = p.qHeads / p.kvHeads;
-  const bool final = part.t0 == 0 && part.t1 == part.tiles;
-  __syncwarp();
-  for (; redo; redo &= redo - 1) {
-    const int x = (threadIdx.x & 96) + __ffs(redo) - 1;
-    const int r = mTile * BM + x, node = r / heads, head = part.kvh * heads + r - node * heads;
-    const TreeRow row = tree_row(p, part.b, node, part.rows, part.nodes);
-    float a[4], m, l;
-    exact_tree_row(p, part, node, head, row, a, m, l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    __half* out = static_cast<__half*>(p.out) + (((int64_t)part.b * p.nodes + node) * p.qHeads + head) * p.hd;
+// The marked rows of a run, key by key: at the block's end, by all of its warps and where nobody waits for them.  (Between a
+// warpgroup's parts, by the warp whose rows they were, they took longer than the waits of its stream may.)  256 rows of 8 heads
+// over 65001 keys: 18 ms.
+__device__ __noinline__ void redo_rows(const TreeParams& p, const Plan& plan, int columns, int group, int mTile) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = p.qHeads / p.kvHeads;
+  Walk walk;
+  walk.begin(p, plan, group);
+  for (int index = 0; walk.next(p, plan); walk.advance(), index++) {
+    const Part part = walk.part();
+    if (part.t0 == part.t1) continue;
+    const bool final = part.t0 == 0 && part.t1 == part.tiles;
+    const int shift = columns != p.hd && !plan.heads4 ? (part.kvh * p.hd) & 7 : 0;
+    const int64_t place = ((int64_t)group * 2 + (index > 0 ? 1 : 0)) * plan.mTiles + mTile;
+    float* const acc = plan.acc + place * (columns * BM);
+    float* const ml = plan.ml + place * (2 * BM);
+    for (int x = warp; x < BM; x += kThreads / 32) {
+      const int r = mTile * BM + x, node = r / heads, head = part.kvh * heads + r - node * heads;
+      if (node >= part.nodes) break;
+      __half* out = static_cast<__half*>(p.out) + (((int64_t)part.b * p.nodes + node) * p.qHeads + head) * p.hd;
+      if (final ? *reinterpret_cast<const unsigned short*>(out) != kAgain : __float_as_uint(ml[2 * x + 1]) != kAgainSum) continue;
+      const TreeRow row = tree_row(p, part.b, node, part.rows, part.nodes);
+      float a[4], m, l;
+      exact_tree_row(p, part, node, head, row, a, m, l);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const int col = lane + 32 * c;
-      if (col >= p.hd) continue;
-      if (final) out[col] = __float2half_rn(a[c] * inv);
-      else acc[((col + shift) / 4 * BM + x) * 4 + (col + shift) % 4] = a[c];
+      for (int c = 0; c < 4; c++) {
+        const int col = lane + 32 * c;
+        if (col >= p.hd) continue;
+        if (final) out[col] = __float2half_rn(a[c] * inv);
+        else acc[((col + shift) / 4 * BM + x) * 4 + (col + shift) % 4] = a[c];
+      }
+      if (!final && lane == 0) ml[2 * x] = m, ml[2 * x + 1] = l;
     }
-    if (!final && lane == 0) ml[2 * x] = m, ml[2 * x + 1] = l;
   }
 }
 
@@ -526,6 +582,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
 
   if (tid == 0) {
     sh.abort = (sQ & 1023u) != 0;   // (there is no static shared memory before it)
+    sh.marked[0] = sh.marked[1] = 0;
     for (int i = 0; i < kMaxSlots; i++) {
       mbar_init(bar(sh.kFull[i]), 1);
       mbar_init(bar(sh.kEmpty[i]), consumers);
@@ -867,8 +924,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
         float* const acc = plan.acc + place * (HD * BM);
         float* const ml = plan.ml + place * (2 * BM);
         const bool odd = (*spoilt & row.nodes) || *spoiltRow >= row.lo;
-        const uint32_t redo = store_rows<HD, PADDED>(p, part, node, head, here, shift, oCol, seen, l, odd, acc, ml);
-        if (redo) redo_rows(p, part, mTile, shift, redo, acc, ml);
+        if (store_rows<HD, PADDED>(p, part, node, head, here, shift, oCol, seen, l, odd, !PADDED || plan.heads4, acc, ml))
+          sh.marked[g] = 1;
       }
       if (!plan.whole && mTile == 0 && rowInTile == 0) {
         int2* const join = plan.joins + (int64_t)part.b * p.kvHeads + part.kvh;
@@ -889,6 +946,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__
     wait_for_what_is_asked(sh, nK, nV);
     if (tid == 0) atomicOr(p.status, kStatusWaitTimeout);
     __syncthreads();
+  } else if (sh.marked[0] | sh.marked[1]) {
+    for (int g = 0; g < 2; g++)
+      if (sh.marked[g]) redo_rows(p, plan, HD, run_of(g), tile_of(g));
   }
   if (warp == 9) {
     tc_fence_after_sync();
