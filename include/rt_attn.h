@@ -626,6 +626,13 @@ typedef struct {
   int32_t indexStride;      /* elements between the sequences' indices; 0 = nodes */
 } rt_commit_args;
 RT_API int rt_commit_rows(rt_ctx* ctx, const rt_commit_args* args);
+/* The same, and committed[b] becomes the number of rows that sequence b got: lead + counts[b], or 0
+ * where it was left alone.  That is what its length grows by.  committed overlaps no other tensor. */
+typedef struct {
+  rt_commit_args commit;
+  int32_t* committed;       /* device [batch] */
+} rt_commit_counted_args;
+RT_API int rt_commit_rows_counted(rt_ctx* ctx, const rt_commit_counted_args* args);
 
 #ifdef __cplusplus
 }

@@ -115,6 +115,9 @@ VerifyArgs = _struct("VerifyArgs", "rt_verify_args.",
 CommitArgs = _struct("CommitArgs", "rt_commit_args.",
                      "A:caches,fresh P:index,counts,kvLens q:cacheSeqStride,freshRowStride,width "
                      "i:dtype,tensors,batch,nodes,cacheRows,lead,indexStride")
+CommitCountedArgs = _struct("CommitCountedArgs", "rt_commit_counted_args, rt_commit_args' fields first.",
+                            "A:caches,fresh P:index,counts,kvLens q:cacheSeqStride,freshRowStride,width "
+                            "i:dtype,tensors,batch,nodes,cacheRows,lead,indexStride P:committed")
 
 
 # name -> (restype, argtypes); every symbol include/rt_attn.h declares.
@@ -166,6 +169,7 @@ SYMBOLS = {
     "rt_attn_tree_route": (C.c_int, [C.c_void_p, C.POINTER(TreeArgs), C.POINTER(C.c_char_p)]),
     "rt_verify_drafts": (C.c_int, [C.c_void_p, C.POINTER(VerifyArgs)]),
     "rt_commit_rows": (C.c_int, [C.c_void_p, C.POINTER(CommitArgs)]),
+    "rt_commit_rows_counted": (C.c_int, [C.c_void_p, C.POINTER(CommitCountedArgs)]),
 }
 
 # What csrc/host.cpp calls, in the order of its table.

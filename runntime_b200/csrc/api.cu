@@ -1026,9 +1026,7 @@ int rt_verify_drafts(rt_ctx* ctx, const rt_verify_args* a) {
   return RT_OK;
 }
 
-int rt_commit_rows(rt_ctx* ctx, const rt_commit_args* a) {
-  RT_ENTER(ctx);
-  if (!a) return fail(ctx, RT_INVALID_ARGUMENT, "rt_commit_rows: args is NULL");
+static int commit_rows(rt_ctx* ctx, const rt_commit_args* a, int32_t* committed) {
   if (!a->caches || !a->fresh || !a->index || !a->counts || !a->kvLens)
     return fail(ctx, RT_INVALID_ARGUMENT, "rt_commit_rows: NULL pointer");
   const int s = check_nodes(ctx, "rt_commit_rows", a->dtype, a->batch, a->nodes);
@@ -1052,10 +1050,23 @@ int rt_commit_rows(rt_ctx* ctx, const rt_commit_args* a) {
     return fail(ctx, RT_INVALID_ARGUMENT, "rt_commit_rows: freshRowStride %lld is smaller than one row",
                 (long long)a->freshRowStride);
   int launches = 0;
-  const cudaError_t e = rt::launch_commit(*a, ctx->status, ctx->smCount, &launches, ctx->stream);
+  const cudaError_t e = rt::launch_commit(*a, committed, ctx->status, ctx->smCount, &launches, ctx->stream);
   ctx->launches += launches;
   RT_CUDA(ctx, e);
   return RT_OK;
+}
+
+int rt_commit_rows(rt_ctx* ctx, const rt_commit_args* a) {
+  RT_ENTER(ctx);
+  if (!a) return fail(ctx, RT_INVALID_ARGUMENT, "rt_commit_rows: args is NULL");
+  return commit_rows(ctx, a, nullptr);
+}
+
+int rt_commit_rows_counted(rt_ctx* ctx, const rt_commit_counted_args* a) {
+  RT_ENTER(ctx);
+  if (!a) return fail(ctx, RT_INVALID_ARGUMENT, "rt_commit_rows: args is NULL");
+  if (!a->committed) return fail(ctx, RT_INVALID_ARGUMENT, "rt_commit_rows: committed is NULL");
+  return commit_rows(ctx, &a->commit, a->committed);
 }
 
 }  // extern "C"

@@ -23,6 +23,7 @@ struct Params {
   const int32_t* counts;
   const int32_t* kvLens;
   int64_t cacheSeqStride, freshSeqStride, freshRowStride, width;   // in units of the copies
+  int32_t* committed;
   int* status;
   int32_t nodes, cacheRows, lead, indexStride;
 };
@@ -44,7 +45,9 @@ __global__ void __launch_bounds__(kThreads) commit_kernel(const __grid_constant_
     pick += p.lead;
   }
   if (j < p.nodes) from[j] = pick;
-  if (__syncthreads_or(bad)) {
+  const bool refused = __syncthreads_or(bad);
+  if (p.committed && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) p.committed[b] = refused ? 0 : (int32_t)n;
+  if (refused) {
     if (threadIdx.x == 0) atomicOr(p.status, kStatusBadState);
     return;
   }
@@ -65,7 +68,8 @@ __global__ void __launch_bounds__(kThreads) commit_kernel(const __grid_constant_
 }
 
 template <typename V, int N>
-cudaError_t launch_n(const rt_commit_args& a, int elems, int* status, int smCount, int* launches, cudaStream_t s) {
+cudaError_t launch_n(const rt_commit_args& a, int32_t* committed, int elems, int* status, int smCount, int* launches,
+                     cudaStream_t s) {
   const int64_t rowStride = a.freshRowStride ? a.freshRowStride : a.width;
   for (int first = 0; first < a.tensors; first += N) {
     const int count = a.tensors - first < N ? a.tensors - first : N;
@@ -81,6 +85,7 @@ cudaError_t launch_n(const rt_commit_args& a, int elems, int* status, int smCoun
     p.freshSeqStride = a.nodes * rowStride / elems;
     p.freshRowStride = rowStride / elems;
     p.width = a.width / elems;
+    p.committed = committed;
     p.status = status;
     p.nodes = a.nodes;
     p.cacheRows = a.cacheRows;
@@ -99,24 +104,25 @@ cudaError_t launch_n(const rt_commit_args& a, int elems, int* status, int smCoun
 }
 
 template <typename V>
-cudaError_t launch(const rt_commit_args& a, int elems, int* status, int smCount, int* launches, cudaStream_t s) {
-  return a.tensors <= kFew ? launch_n<V, kFew>(a, elems, status, smCount, launches, s)
-                           : launch_n<V, kTensors>(a, elems, status, smCount, launches, s);
+cudaError_t launch(const rt_commit_args& a, int32_t* committed, int elems, int* status, int smCount, int* launches,
+                   cudaStream_t s) {
+  return a.tensors <= kFew ? launch_n<V, kFew>(a, committed, elems, status, smCount, launches, s)
+                           : launch_n<V, kTensors>(a, committed, elems, status, smCount, launches, s);
 }
 
 }  // namespace
 
-cudaError_t launch_commit(const rt_commit_args& a, int* status, int smCount, int* launches, cudaStream_t s) {
+cudaError_t launch_commit(const rt_commit_args& a, int32_t* committed, int* status, int smCount, int* launches, cudaStream_t s) {
   const int es = a.dtype == RT_F16 ? 2 : 4;
   // The widest copies that every address and stride is a multiple of.
   uintptr_t all = 16 | (uintptr_t)(a.width * es) | (uintptr_t)(a.freshRowStride * es) | (uintptr_t)(a.cacheSeqStride * es);
   for (int t = 0; t < a.tensors; t++)
     all |= reinterpret_cast<uintptr_t>(a.caches[t]) | reinterpret_cast<uintptr_t>(a.fresh[t]);
   const int bytes = (int)(all & (~all + 1));
-  if (bytes == 16) return launch<uint4>(a, 16 / es, status, smCount, launches, s);
-  if (bytes == 8) return launch<uint2>(a, 8 / es, status, smCount, launches, s);
-  if (bytes == 4) return launch<uint32_t>(a, 4 / es, status, smCount, launches, s);
-  return launch<uint16_t>(a, 1, status, smCount, launches, s);
+  if (bytes == 16) return launch<uint4>(a, committed, 16 / es, status, smCount, launches, s);
+  if (bytes == 8) return launch<uint2>(a, committed, 8 / es, status, smCount, launches, s);
+  if (bytes == 4) return launch<uint32_t>(a, committed, 4 / es, status, smCount, launches, s);
+  return launch<uint16_t>(a, committed, 1, status, smCount, launches, s);
 }
 
 }  // namespace rt

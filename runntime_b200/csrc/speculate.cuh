@@ -92,6 +92,7 @@ cudaError_t launch_tree_tc(const TreeParams& p, int smCount, bool whole, int* la
 
 cudaError_t launch_rotary(const rt_rotary_args& a, int smCount, cudaStream_t s);
 cudaError_t launch_verify(const rt_verify_args& a, int* status, int smCount, cudaStream_t s);
-cudaError_t launch_commit(const rt_commit_args& a, int* status, int smCount, int* launches, cudaStream_t s);
+// committed (or NULL): the rows that each sequence got.
+cudaError_t launch_commit(const rt_commit_args& a, int32_t* committed, int* status, int smCount, int* launches, cudaStream_t s);
 
 }  // namespace rt

@@ -31,7 +31,7 @@ import ctypes as C
 import math
 from typing import Optional, Sequence, Tuple
 
-from ._lib import (AttnArgs, CommitArgs, DecodeArgs, DecodeSecond, DTYPE_CODE, Exchange, MAX_NODES,
+from ._lib import (AttnArgs, CommitArgs, CommitCountedArgs, DecodeArgs, DecodeSecond, DTYPE_CODE, Exchange, MAX_NODES,
                    MAX_ROTARY_WINDOWS, RotaryArgs, TreeArgs, VerifyArgs, WINDOW_INF, call, check)
 from .executor import CudaExecutor
 
@@ -274,18 +274,23 @@ def verify_batched(ex: CudaExecutor, target, tokens, accept, sample, path, outTo
 def commit_batched(ex: CudaExecutor, caches: Sequence, fresh: Sequence, index, counts, kvLens, *, dtype: str,
                    batch: int, nodes: int, cacheRows: int, width: int, lead: int = 0,
                    cacheSeqStride: Optional[int] = None, freshRowStride: int = 0,
-                   indexStride: int = 0) -> None:
+                   indexStride: int = 0, committed=None) -> None:
     """Rows of the tokens that stand into the caches, by rt_commit_rows (include/rt_attn.h): for every tensor of
     ``caches`` (K and V of all layers, [batch, cacheRows, width] each: a sequence of them or one tensor) rows
     ``kvLens[b]``... become rows 0..lead-1 and lead + ``index[b][j]``, j < ``counts[b]``, of its [batch*nodes, width]
     tensor in ``fresh``.
-    ``index`` and ``counts`` are verify_batched's ``path`` and ``accepted``; ``kvLens`` is not advanced."""
+    ``index`` and ``counts`` are verify_batched's ``path`` and ``accepted``; ``kvLens`` is not advanced.  ``committed``
+    (device int32 [batch]) becomes what each sequence's length grows by: 0 for one that was left alone."""
     n = len(caches)
     if n != len(fresh):
         raise ValueError(f"commit: {n} caches and {len(fresh)} tensors of new rows")
-    call(ex._lib, "rt_commit_rows", ex.ctx, CommitArgs, _each(caches), _each(fresh), index, counts, kvLens,
-         cacheRows * width if cacheSeqStride is None else cacheSeqStride, freshRowStride, width, DTYPE_CODE[dtype], n,
-         batch, nodes, cacheRows, lead, indexStride)
+    values = (_each(caches), _each(fresh), index, counts, kvLens,
+              cacheRows * width if cacheSeqStride is None else cacheSeqStride, freshRowStride, width, DTYPE_CODE[dtype], n,
+              batch, nodes, cacheRows, lead, indexStride)
+    if committed is None:
+        call(ex._lib, "rt_commit_rows", ex.ctx, CommitArgs, *values)
+    else:
+        call(ex._lib, "rt_commit_rows_counted", ex.ctx, CommitCountedArgs, *values, committed)
 
 
 def _each(tensors):
@@ -316,6 +321,7 @@ class KvCacheEngine:
         self.k = torch.zeros(batch, maxPositions, kvw, dtype=tdt, device=dev)
         self.v = torch.zeros(batch, maxPositions, kvw, dtype=tdt, device=dev)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.committed = torch.zeros_like(self.lens)      # rows of the last commitTree
         self.maxLen, self.exact = 0, True     # the longest sequence, or a bound of it
         self.cross: Optional[Tuple[object, object, int]] = None
         self.rope = None
@@ -430,15 +436,15 @@ class KvCacheEngine:
         ``accepted``) go to the ends of the caches, and the lengths grow by them.  With lead = 1 node 0 is the
         token that the last step ended with and the others are the verified ones, nodes - 1 to a row of
         ``index`` unless indexStride says otherwise.  Every sequence gets its ``lead`` rows; where some have
-        ended, lead = 0 with all of a sequence's rows in ``index``, none of an ended one."""
+        ended, lead = 0 with all of a sequence's rows in ``index``, none of an ended one.  A sequence whose rows do
+        not fit or whose indices are out of range is left as it is, its length too (``committed`` 0), and the
+        executor's sync reports it."""
         _bind_to_torch_stream(self.ex)
         commit_batched(self.ex, (self.k, self.v), (kNew, vNew), index, accepted, self.lens, dtype=self.dtype,
                        batch=self.batch, nodes=nodes, cacheRows=self.maxPositions,
                        width=self.kvHeads * self.headDim, lead=lead, freshRowStride=freshRowStride,
-                       indexStride=indexStride or max(nodes - lead, 1))
-        self.lens.add_(accepted)
-        if lead:
-            self.lens.add_(lead)
+                       indexStride=indexStride or max(nodes - lead, 1), committed=self.committed)
+        self.lens.add_(self.committed)
         self.maxLen, self.exact = min(self.maxLen + nodes, self.maxPositions), False
 
     def commitTreeQkv(self, qkv, index, accepted, *, nodes: int, lead: int = 1, indexStride: int = 0) -> None:
