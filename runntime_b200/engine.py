@@ -422,7 +422,7 @@ class KvCacheEngine:
         width, es, base = qw + 2 * kvw, qkv.element_size(), qkv.data_ptr()
         _bind_to_torch_stream(self.ex)
         self._room(nodes)
-        positions = self.lens[:, None] + depths
+        positions = (self.lens[:, None] + depths).contiguous()   # (a sum has its operands' order in memory)
         rotary_batched(self.ex, base, positions, plan,
                        [(0, self.qHeads, base, width), (qw, self.kvHeads, base + qw * es, width)], dtype=self.dtype,
                        rows=self.batch * nodes, headDim=self.headDim, layout=layout, xRowStride=width)

@@ -1,7 +1,51 @@
 """KvCacheEngine's speculative step without a GPU: the structures of its calls, and what it refuses before them."""
 import ctypes as C
 
+import pytest
+
 import runntime_b200._lib as L
+from runntime_b200 import engine
+
+
+@pytest.fixture
+def step(monkeypatch):
+    """An engine of three sequences on the CPU, and what its calls would be given."""
+    torch = pytest.importorskip("torch")
+    seen = []
+
+    def rotary(ex, x, positions, plan, windows, **more):
+        assert positions.dtype == torch.int32 and positions.numel() >= more["rows"]
+        # what the kernel reads: rows numbers from the first address on
+        seen.append(positions.as_strided((more["rows"],), (1,), positions.storage_offset()).tolist())
+
+    monkeypatch.setattr(engine, "_bind_to_torch_stream", lambda ex: None)
+    monkeypatch.setattr(engine, "rotary_batched", rotary)
+    monkeypatch.setattr(engine, "tree_batched", lambda *a, **k: None)
+    eng = engine.KvCacheEngine(None, batch=3, maxPositions=64, qHeads=2, kvHeads=1, headDim=8, device="cpu")
+    eng.lens.copy_(torch.tensor([10, 20, 30]))
+    eng.maxLen = 30
+    eng.qkv = torch.zeros(12, 32, dtype=torch.float16)
+
+    def call(depths, qkv=None):
+        eng.stepTreeQkv(eng.qkv if qkv is None else qkv, None, None, depths, nodes=4)
+        return seen[-1]
+
+    call.engine, call.seen = eng, seen
+    return call
+
+
+def test_positions_are_rows_one_after_the_other(step):
+    """Depths in any order in memory: the positions lie sequence by sequence."""
+    torch = pytest.importorskip("torch")
+    step.engine.setRotary(engine.RotaryPlan(8, None, 1.0))
+    depths = torch.tensor([[0, 1, 1, 2], [0, 1, 2, 3], [0, 0, 1, 1]], dtype=torch.int32)
+    want = [a + d for a, ds in zip((10, 20, 30), depths.tolist()) for d in ds]
+    assert step(depths) == want
+    assert step(depths.t().contiguous().t()) == want          # kept as [nodes, batch]
+    assert step(depths.repeat_interleave(2, 1)[:, ::2]) == want
+    for one in (depths[0], depths[:1], depths[0].expand(3, 4)):
+        assert step(one) == [a + d for a in (10, 20, 30) for d in depths[0].tolist()]
+
 
 
 def test_counted_commit_is_a_commit_and_an_address():
