@@ -415,9 +415,14 @@ class KvCacheEngine:
         q|k|v): q and k are turned in place by setRotary's plan at the sequence's length plus ``depths``
         (device int32 [nodes] or [batch, nodes]).  qkv then holds the keys and values that
         commitTreeQkv takes."""
+        if self.rotary is None:
+            raise ValueError("stepTreeQkv: setRotary has not been called")
         plan, layout = self.rotary
         if depths.dtype != self.lens.dtype:
             raise ValueError(f"stepTreeQkv: depths are {depths.dtype}, not {self.lens.dtype}")
+        if tuple(depths.shape) not in ((nodes,), (1, nodes), (self.batch, nodes)):
+            raise ValueError(f"stepTreeQkv: depths of shape {tuple(depths.shape)} are neither [{nodes}] nor "
+                             f"[{self.batch}, {nodes}]")
         qw, kvw = self.qHeads * self.headDim, self.kvHeads * self.headDim
         width, es, base = qw + 2 * kvw, qkv.element_size(), qkv.data_ptr()
         _bind_to_torch_stream(self.ex)

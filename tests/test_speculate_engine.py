@@ -47,6 +47,22 @@ def test_positions_are_rows_one_after_the_other(step):
         assert step(one) == [a + d for a in (10, 20, 30) for d in depths[0].tolist()]
 
 
+def test_depths_of_another_shape_are_refused(step):
+    torch = pytest.importorskip("torch")
+    step.engine.setRotary(engine.RotaryPlan(8, None, 1.0))
+    for shape in ((1,), (3,), (5,), (3, 1), (3, 3), (1, 3), (2, 4), (4, 3), (3, 5), (), (1, 3, 4)):
+        with pytest.raises(ValueError, match="depths of shape"):
+            step(torch.zeros(shape, dtype=torch.int32))
+    with pytest.raises(ValueError, match="depths are torch.int64"):
+        step(torch.zeros(4, dtype=torch.int64))
+    assert not step.seen
+
+
+def test_a_step_without_frequencies_is_refused(step):
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError, match="setRotary"):
+        step(torch.zeros(4, dtype=torch.int32))
+
 
 def test_counted_commit_is_a_commit_and_an_address():
     assert L.CommitCountedArgs.layout == L.CommitArgs.layout + "P"
