@@ -302,6 +302,22 @@ def _each(tensors):
     return range(base, base + len(tensors) * step, step) if step else [base] * len(tensors)
 
 
+def _check_ints(call: str, name: str, x, kind: str, rows: int, cols: int, stride: int) -> None:
+    """Refuses a tensor that does not hold what a kernel reads from its address on: ``rows`` times ``cols`` integers
+    of ``kind``, ``stride`` elements from one row to the next.  Addresses are taken as they are."""
+    if not hasattr(x, "dtype"):
+        return
+    if str(x.dtype) != "torch." + kind:
+        raise ValueError(f"{call}: {name} is {x.dtype}, not torch.{kind}")
+    if x.is_contiguous() and (x.dim() != 2 or rows == 1 or x.shape[1] == stride):
+        fits = cols == 0 or x.numel() >= (rows - 1) * stride + cols
+    else:
+        fits = cols == 0 or x.dim() == 2 and x.shape[0] >= rows and x.shape[1] >= cols and x.stride() == (stride, 1)
+    if not fits:
+        raise ValueError(f"{call}: {name} of shape {tuple(x.shape)} and strides {tuple(x.stride())} does not hold {rows} rows "
+                         f"of {cols}, {stride} elements apart")
+
+
 class KvCacheEngine:
     """Preallocated self-attention caches for ``batch`` sequences plus their
     lengths, stepped one token at a time: append + causal attend in one kernel.
@@ -444,11 +460,14 @@ class KvCacheEngine:
         ended, lead = 0 with all of a sequence's rows in ``index``, none of an ended one.  A sequence whose rows do
         not fit or whose indices are out of range is left as it is, its length too (``committed`` 0), and the
         executor's sync reports it."""
+        stride = indexStride or max(nodes - lead, 1)
+        _check_ints("commitTree", "accepted", accepted, "int32", 1, self.batch, self.batch)
+        _check_ints("commitTree", "index", index, "int32", self.batch, max(nodes - lead, 0), stride)
         _bind_to_torch_stream(self.ex)
         commit_batched(self.ex, (self.k, self.v), (kNew, vNew), index, accepted, self.lens, dtype=self.dtype,
                        batch=self.batch, nodes=nodes, cacheRows=self.maxPositions,
                        width=self.kvHeads * self.headDim, lead=lead, freshRowStride=freshRowStride,
-                       indexStride=indexStride or max(nodes - lead, 1), committed=self.committed)
+                       indexStride=stride, committed=self.committed)
         self.lens.add_(self.committed)
         self.maxLen, self.exact = min(self.maxLen + nodes, self.maxPositions), False
 

@@ -69,3 +69,54 @@ def test_counted_commit_is_a_commit_and_an_address():
     assert L.CommitCountedArgs.committed.offset == C.sizeof(L.CommitArgs)
     for name, _ in L.CommitArgs._fields_:
         assert getattr(L.CommitCountedArgs, name).offset == getattr(L.CommitArgs, name).offset
+
+
+@pytest.fixture
+def commit(monkeypatch):
+    """commitTree of an engine of three sequences on the CPU, with what its call would be given."""
+    torch = pytest.importorskip("torch")
+    seen = []
+    monkeypatch.setattr(engine, "_bind_to_torch_stream", lambda ex: None)
+    monkeypatch.setattr(engine, "commit_batched", lambda ex, caches, fresh, index, counts, lens, **more: seen.append(more))
+    eng = engine.KvCacheEngine(None, batch=3, maxPositions=64, qHeads=2, kvHeads=1, headDim=8, device="cpu")
+
+    def call(index, accepted, nodes=5, **more):
+        eng.commitTree(0, 0, index, accepted, nodes=nodes, **more)
+        return seen.pop()
+
+    call.seen = seen
+    call.ints = lambda *shape, dtype=torch.int32: torch.zeros(shape, dtype=dtype)
+    return call
+
+
+def test_indices_and_counts_that_a_commit_takes(commit):
+    z = commit.ints
+    assert commit(z(3, 4), z(3))["indexStride"] == 4
+    assert commit(z(12), z(3))["indexStride"] == 4
+    assert commit(z(3, 5), z(3), lead=0)["indexStride"] == 5
+    assert commit(z(3, 9), z(3), indexStride=9)["indexStride"] == 9
+    assert commit(z(3, 9)[:, :4], z(3), indexStride=9)["indexStride"] == 9
+    assert commit(z(3, 9)[:, 2:6], z(4)[1:], indexStride=9)["indexStride"] == 9
+    assert commit(z(3, 1), z(3), nodes=1)["indexStride"] == 1      # the leading rows alone
+    assert commit(z(4, 4)[1:], z(3))["indexStride"] == 4
+    assert commit(12345, 678)["indexStride"] == 4                  # addresses
+
+
+def test_indices_and_counts_that_a_commit_refuses(commit):
+    """64-bit numbers would be read as twice as many of 32 bits, rows further apart as rows of other sequences."""
+    torch = pytest.importorskip("torch")
+    z = commit.ints
+    for bad, match in (((z(3, 4), z(3, dtype=torch.int64)), "accepted is torch.int64"),
+                       ((z(3, 4, dtype=torch.int64), z(3)), "index is torch.int64"),
+                       ((z(3, 4), z(3, dtype=torch.float32)), "accepted is torch.float32"),
+                       ((z(3, 4), z(2)), "accepted of shape"), ((z(3, 4), z(6)[::2]), "accepted of shape"),
+                       ((z(3, 3), z(3)), "index of shape"), ((z(2, 4), z(3)), "index of shape"),
+                       ((z(3, 7), z(3)), "index of shape"), ((z(3, 8)[:, ::2], z(3)), "index of shape"),
+                       ((z(4, 3).t(), z(3)), "index of shape"), ((z(11), z(3)), "index of shape")):
+        with pytest.raises(ValueError, match=match):
+            commit(*bad)
+    with pytest.raises(ValueError, match="index of shape"):
+        commit(z(3, 4), z(3), lead=0)
+    with pytest.raises(ValueError, match="index of shape"):
+        commit(z(3, 9), z(3), indexStride=8)
+    assert not commit.seen
