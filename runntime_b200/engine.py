@@ -302,11 +302,13 @@ def _each(tensors):
     return range(base, base + len(tensors) * step, step) if step else [base] * len(tensors)
 
 
-def _check_ints(call: str, name: str, x, kind: str, rows: int, cols: int, stride: int) -> None:
-    """Refuses a tensor that does not hold what a kernel reads from its address on: ``rows`` times ``cols`` integers
+def _check_tensor(call: str, name: str, x, kind: str, device, rows: int, cols: int, stride: int) -> None:
+    """Refuses a tensor that does not hold what a kernel reads from its address on: ``rows`` times ``cols`` numbers
     of ``kind``, ``stride`` elements from one row to the next.  Addresses are taken as they are."""
     if not hasattr(x, "dtype"):
         return
+    if x.device != device:
+        raise ValueError(f"{call}: {name} is on {x.device}, not on {device}")
     if str(x.dtype) != "torch." + kind:
         raise ValueError(f"{call}: {name} is {x.dtype}, not torch.{kind}")
     if x.is_contiguous() and (x.dim() != 2 or rows == 1 or x.shape[1] == stride):
@@ -417,6 +419,10 @@ class KvCacheEngine:
                  qRowStride: int = 0, kNewRowStride: int = 0, vNewRowStride: int = 0, sinks=None) -> None:
         """``nodes`` drafted tokens of every sequence attend to its cache and to their ancestors
         (tree_batched).  Nothing is appended: commitTree does that for the tokens that stand."""
+        device = self.lens.device
+        _check_tensor("stepTree", "masks", masks, "int64", device, 1 if sharedMasks else self.batch, nodes, nodes)
+        _check_tensor("stepTree", "nodeCounts", nodeCounts, "int32", device, 1, self.batch, self.batch)
+        _check_tensor("stepTree", "sinks", sinks, "float32", device, 1, self.qHeads, self.qHeads)
         _bind_to_torch_stream(self.ex)
         self._room(nodes)
         tree_batched(self.ex, q, out, self.k, self.v, kNew, vNew, masks, dtype=self.dtype, batch=self.batch,
@@ -461,8 +467,9 @@ class KvCacheEngine:
         not fit or whose indices are out of range is left as it is, its length too (``committed`` 0), and the
         executor's sync reports it."""
         stride = indexStride or max(nodes - lead, 1)
-        _check_ints("commitTree", "accepted", accepted, "int32", 1, self.batch, self.batch)
-        _check_ints("commitTree", "index", index, "int32", self.batch, max(nodes - lead, 0), stride)
+        device = self.lens.device
+        _check_tensor("commitTree", "accepted", accepted, "int32", device, 1, self.batch, self.batch)
+        _check_tensor("commitTree", "index", index, "int32", device, self.batch, max(nodes - lead, 0), stride)
         _bind_to_torch_stream(self.ex)
         commit_batched(self.ex, (self.k, self.v), (kNew, vNew), index, accepted, self.lens, dtype=self.dtype,
                        batch=self.batch, nodes=nodes, cacheRows=self.maxPositions,

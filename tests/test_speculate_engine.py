@@ -120,3 +120,37 @@ def test_indices_and_counts_that_a_commit_refuses(commit):
     with pytest.raises(ValueError, match="index of shape"):
         commit(z(3, 9), z(3), indexStride=8)
     assert not commit.seen
+
+
+def test_masks_counts_and_sinks_that_a_step_takes_and_refuses(monkeypatch):
+    torch = pytest.importorskip("torch")
+    seen = []
+    monkeypatch.setattr(engine, "_bind_to_torch_stream", lambda ex: None)
+    monkeypatch.setattr(engine, "tree_batched", lambda *a, **k: seen.append(k))
+    eng = engine.KvCacheEngine(None, batch=3, maxPositions=64, qHeads=4, kvHeads=2, headDim=8, device="cpu")
+
+    def call(masks, **more):
+        eng.stepTree(0, 0, 0, 0, masks, nodes=5, **more)
+        seen.pop()
+
+    def z(*shape, dtype=torch.int64):
+        return torch.zeros(shape, dtype=dtype)
+
+    i32, f32 = torch.int32, torch.float32
+    call(z(3, 5))
+    call(z(15))
+    call(z(5), sharedMasks=True)
+    call(z(3, 5), sharedMasks=True)
+    call(z(5, 5)[1:4], nodeCounts=z(3, dtype=i32), sinks=z(4, dtype=f32))
+    call(123, nodeCounts=456, sinks=789)
+    for masks, more, match in ((z(3, 5, dtype=i32), {}, "masks is torch.int32"), (z(5), {}, "masks of shape"),
+                               (z(3, 7), {}, "masks of shape"), (z(5, 3).t(), {}, "masks of shape"), (z(2, 5), {}, "masks of shape"),
+                               (z(4), dict(sharedMasks=True), "masks of shape"),
+                               (z(5).to("meta"), dict(sharedMasks=True), "masks is on meta"),
+                               (z(3, 5), dict(nodeCounts=z(3)), "nodeCounts is torch.int64"),
+                               (z(3, 5), dict(nodeCounts=z(2, dtype=i32)), "nodeCounts of shape"),
+                               (z(3, 5), dict(sinks=z(4, dtype=torch.float16)), "sinks is torch.float16"),
+                               (z(3, 5), dict(sinks=z(2, dtype=f32)), "sinks of shape")):
+        with pytest.raises(ValueError, match=match):
+            call(masks, **more)
+    assert not seen
