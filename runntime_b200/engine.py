@@ -180,7 +180,8 @@ def rotary_frequencies(rotaryDim: int, *, base: float = 10000.0,
 
 def rotary_plan(rotaryDim: int, *, base: float = 10000.0, scaling: Optional[dict] = None,
                 device=None) -> RotaryPlan:
-    """The plan of rotary_batched for ``rotary_frequencies(rotaryDim, base=base, scaling=scaling)``."""
+    """The plan of rotary_batched for ``rotary_frequencies(rotaryDim, base=base, scaling=scaling)``, on ``device`` (the
+    executor's; torch's default device, which is the CPU as a rule, if None)."""
     import torch
     f, scale = rotary_frequencies(rotaryDim, base=base, scaling=scaling)
     turns = [int(x / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for x in f]
@@ -204,6 +205,8 @@ def rotary_batched(ex: CudaExecutor, x, positions, plan: RotaryPlan, windows: Se
     n = len(windows)
     if not 1 <= n <= MAX_ROTARY_WINDOWS:
         raise ValueError(f"rotary: takes 1..{MAX_ROTARY_WINDOWS} windows, got {n}")
+    if getattr(plan.turns, "is_cuda", True) is False:
+        raise ValueError(f"rotary: the plan is on {plan.turns.device}: rotary_plan's device is the executor's")
     flat = []
     for w in windows:
         flat += (w[0], w[2], w[3] if len(w) > 3 else 0, w[1], 0)

@@ -154,3 +154,11 @@ def test_masks_counts_and_sinks_that_a_step_takes_and_refuses(monkeypatch):
         with pytest.raises(ValueError, match=match):
             call(masks, **more)
     assert not seen
+
+
+def test_a_plan_in_host_memory_is_refused():
+    """rotary_plan's default device is torch's; a kernel cannot read from the CPU's."""
+    pytest.importorskip("torch")
+    for plan in (engine.rotary_plan(8), engine.rotary_plan(8, device="cpu")):
+        with pytest.raises(ValueError, match="the plan is on cpu"):
+            engine.rotary_batched(None, 16, 16, plan, [(0, 1, 16)], dtype="f16", rows=1, headDim=8, xRowStride=8)
