@@ -414,6 +414,11 @@ class KvCacheEngine:
                        headDim=self.headDim, kvLen=self.maxLen, kvLens=self.lens, kNew=kNew,
                        vNew=vNew, windowLeft=self.windowLeft, second=sec)
 
+    def _check_qkv(self, call: str, qkv, nodes: int) -> None:
+        width = (self.qHeads + 2 * self.kvHeads) * self.headDim
+        _check_tensor(call, "qkv", qkv, "float16" if self.dtype == "f16" else "float32", self.lens.device, self.batch * nodes,
+                      width, width)
+
     def setRotary(self, plan: RotaryPlan, layout: str = "interleaved") -> None:
         """Frequencies of stepTreeQkv's rotary positions."""
         self.rotary = (plan, layout)
@@ -450,6 +455,7 @@ class KvCacheEngine:
                              f"[{self.batch}, {nodes}]")
         qw, kvw = self.qHeads * self.headDim, self.kvHeads * self.headDim
         width, es, base = qw + 2 * kvw, qkv.element_size(), qkv.data_ptr()
+        self._check_qkv("stepTreeQkv", qkv, nodes)
         _bind_to_torch_stream(self.ex)
         self._room(nodes)
         positions = (self.lens[:, None] + depths).contiguous()   # (a sum has its operands' order in memory)
@@ -484,6 +490,7 @@ class KvCacheEngine:
     def commitTreeQkv(self, qkv, index, accepted, *, nodes: int, lead: int = 1, indexStride: int = 0) -> None:
         """commitTree from the rows that stepTreeQkv has turned."""
         qw, kvw = self.qHeads * self.headDim, self.kvHeads * self.headDim
+        self._check_qkv("commitTreeQkv", qkv, nodes)
         es, base = qkv.element_size(), qkv.data_ptr()
         self.commitTree(base + qw * es, base + (qw + kvw) * es, index, accepted, nodes=nodes, lead=lead,
                         freshRowStride=qw + 2 * kvw, indexStride=indexStride)

@@ -162,3 +162,30 @@ def test_a_plan_in_host_memory_is_refused():
     for plan in (engine.rotary_plan(8), engine.rotary_plan(8, device="cpu")):
         with pytest.raises(ValueError, match="the plan is on cpu"):
             engine.rotary_batched(None, 16, 16, plan, [(0, 1, 16)], dtype="f16", rows=1, headDim=8, xRowStride=8)
+
+
+def test_projections_of_another_type_or_layout_are_refused(step, monkeypatch):
+    """Their rows are turned where they lie: in rows further apart, or of another type, that would be other memory."""
+    torch = pytest.importorskip("torch")
+    eng = step.engine
+    eng.setRotary(engine.RotaryPlan(8, None, 1.0))
+    depths = torch.zeros(4, dtype=torch.int32)
+    committed = []
+    monkeypatch.setattr(engine, "commit_batched", lambda *a, **k: committed.append(k))
+
+    def commit(qkv):
+        eng.commitTreeQkv(qkv, 0, 0, nodes=4)
+
+    good = torch.zeros(12, 32, dtype=torch.float16)
+    for qkv in (good, good.view(3, 4, 32), torch.zeros(13, 32, dtype=torch.float16)[1:]):
+        step(depths, qkv)
+        commit(qkv)
+    assert len(step.seen) == len(committed) == 3
+    for bad, match in ((good.float(), "qkv is torch.float32"), (torch.zeros(12, 64, dtype=torch.float16)[:, :32], "qkv of shape"),
+                       (torch.zeros(32, 12, dtype=torch.float16).t(), "qkv of shape"), (good[:11], "qkv of shape"),
+                       (torch.zeros(12, 40, dtype=torch.float16), "qkv of shape"), (good.to("meta"), "qkv is on meta")):
+        with pytest.raises(ValueError, match="stepTreeQkv: " + match):
+            step(depths, bad)
+        with pytest.raises(ValueError, match="commitTreeQkv: " + match):
+            commit(bad)
+    assert len(step.seen) == len(committed) == 3
