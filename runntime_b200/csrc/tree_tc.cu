@@ -1087,7 +1087,7 @@ Plan plan_of(const TreeParams& p, int smCount, bool whole) {
 }
 
 template <int HD, bool PADDED>
-cudaError_t launch(const TreeParams& p, Plan& plan, cudaStream_t s, std::string* err) {
+cudaError_t launch(const TreeParams& p, Plan& plan, int smCount, cudaStream_t s, std::string* err) {
   CUtensorMap k, v, kn, vn, q;
   // Q by TMA where its rows allow that and a row tile is whole nodes: heads of the group, then nodes, are its rows.
   const int heads = p.qHeads / p.kvHeads;
@@ -1116,7 +1116,7 @@ cudaError_t launch(const TreeParams& p, Plan& plan, cudaStream_t s, std::string*
   e = launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), smem_bytes<HD>(), s, k, v, kn, vn, q, p, plan);
   if (e != cudaSuccess || plan.whole) return e;
   const int64_t units = (int64_t)p.batch * p.kvHeads * plan.mTiles;
-  const bool wide = units * (HD / 32) >= 2 * 148;
+  const bool wide = units * (HD / 32) >= 2 * smCount;   // blocks of sixteen columns to a thread
   auto merge = wide ? tree_tc_merge_kernel<HD, 16> : tree_tc_merge_kernel<HD, 4>;
   return launch_dependent(merge, dim3((unsigned)p.batch * (HD / (wide ? 32 : 8)), (unsigned)p.kvHeads, (unsigned)plan.mTiles),
                           dim3(256), 0, s, p, plan);
@@ -1147,8 +1147,8 @@ cudaError_t launch_tree_tc(const TreeParams& p, int smCount, bool whole, int* la
   plan.ml = p.scratch + (size_t)plan.groups * 2 * plan.mTiles * hdt * BM;
   plan.joins = reinterpret_cast<int2*>(plan.ml + (size_t)plan.groups * 2 * plan.mTiles * 2 * BM);
   *launches = plan.whole ? 1 : 2;
-  if (hdt == 64) return p.hd == 64 ? launch<64, false>(p, plan, s, err) : launch<64, true>(p, plan, s, err);
-  return p.hd == 128 ? launch<128, false>(p, plan, s, err) : launch<128, true>(p, plan, s, err);
+  if (hdt == 64) return p.hd == 64 ? launch<64, false>(p, plan, smCount, s, err) : launch<64, true>(p, plan, smCount, s, err);
+  return p.hd == 128 ? launch<128, false>(p, plan, smCount, s, err) : launch<128, true>(p, plan, smCount, s, err);
 }
 
 }  // namespace rt
