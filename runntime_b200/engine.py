@@ -379,8 +379,11 @@ class KvCacheEngine:
     def _room(self, rows: int) -> None:
         """``rows`` more have to fit behind the longest sequence.  After commitTree the host knows a bound
         of the lengths alone (how many drafted tokens stood is on the device); where that is too large
-        it asks."""
-        if self.maxLen + rows > self.maxPositions and not self.exact:
+        it asks.  Under a capture it cannot: then the kernels alone refuse what has no room, as they do in every replay."""
+        if self.maxLen + rows > self.maxPositions and not self.exact and rows <= self.maxPositions:
+            if _capturing():
+                self.maxLen = self.maxPositions - rows
+                return
             self.maxLen, self.exact = int(self.lens.max().item()), True
         if self.maxLen + rows > self.maxPositions:
             raise ValueError(
@@ -593,6 +596,11 @@ def _bind_to_torch_stream(ex: CudaExecutor) -> None:
     import torch
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     ex.setStream(raw(ex.device) if raw is not None else torch.cuda.current_stream(ex.device).cuda_stream)
+
+
+def _capturing() -> bool:
+    import torch
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
 
 
 class PeerExchangeDecode:

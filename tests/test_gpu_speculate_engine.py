@@ -77,3 +77,50 @@ def test_committed_rows_of_many_tensors(on_torch):
         on_torch.sync()
     assert committed.tolist() == [3, 0]
     assert torch.equal(caches[:, 0, 6:], fresh.view(130, B, T, w)[:, 0]) and (caches[:, 1] == 0).all()
+
+
+def test_a_step_is_captured_when_the_bound_is_full(on_torch):
+    """The host's bound of the lengths has met the capacity, the lengths have not: they cannot be asked for under a capture,
+    and the step is captured all the same; replays go on until the rows no longer fit, and say so."""
+    import runntime_b200 as rt
+    from runntime_b200 import RunntimeError, engine
+    torch = torch_()
+    T, w, most = 8, 128, 24
+    masks = torch.tensor(engine.tree_masks([-1] + [0] * 7), device="cuda")
+    x = torch.randn(2 * T, w, generator=gen(1), device="cuda").half()
+    index, accepted = torch.zeros(2, T - 1, dtype=torch.int32, device="cuda"), dev([1, 0])
+    outs = []
+    e = rt.CudaExecutor(0)
+    try:
+        engines = [engine.KvCacheEngine(ex, batch=2, maxPositions=most, qHeads=2, kvHeads=2, headDim=64) for ex in (on_torch, e)]
+        for eng in engines:
+            out = torch.empty_like(x)
+            outs.append(out)
+            for _ in range(3):
+                eng.stepTree(x, x, x, out, masks, nodes=T, sharedMasks=True)
+                eng.commitTree(x, x, index, accepted, nodes=T)
+            assert eng.maxLen == most and eng.lens.tolist() == [6, 3]
+        eager, captured = engines
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured.stepTree(x, x, x, outs[1], masks, nodes=T, sharedMasks=True)
+            captured.commitTree(x, x, index, accepted, nodes=T)
+        for _ in range(5):                     # 6 + 2 * 5 = 16: eight more still fit
+            eager.stepTree(x, x, x, outs[0], masks, nodes=T, sharedMasks=True)
+            eager.commitTree(x, x, index, accepted, nodes=T)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(eager.lens, captured.lens) and torch.equal(eager.k, captured.k)
+            # (the captured step is planned for another length: the same numbers added up in another order)
+            assert ((outs[0] - outs[1]).abs() <= 2.0 ** -10 * outs[0].abs() + 2.0 ** -11).all()
+        e.sync()
+        for _ in range(6):                     # the first sequence is full after four of them
+            graph.replay()
+        torch.cuda.synchronize()               # (replays are on torch's stream)
+        with pytest.raises(RunntimeError, match="status"):
+            e.sync()
+        assert captured.lens.tolist() == [24, 14]
+        del graph
+    finally:
+        e.dispose()
