@@ -107,3 +107,38 @@ def test_tree_small_probabilities_add_up(on_torch, shape, splits):
     on_torch.sync()
     check(t, got)
     assert (got.view(t.B, -1)[0] > 0).all() and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("shape", [(8, 2, 128), (4, 4, 64), (8, 8, 52), (4, 2, 33)])
+@pytest.mark.parametrize("nodes,window,splits", [(1, None, 0), (5, None, 0), (64, None, 0), (5, 100, 0), (17, None, 7), (5, 64, 3)])
+def test_tree_meets_every_key_once(on_torch, dtype, shape, nodes, window, splits):
+    """Equal scores, and values that are one in one column: a result says how many of the keys of that column were
+    met, of how many in all."""
+    H, K, D = shape
+    t = Tree(dtype, *shape, nodes, [0, 1, 63, 64, 65, 127, 128, 129, 300, 515, 1000], window=window, seed=nodes)
+    torch, T, B = t.torch, nodes, t.B
+    t.q.zero_()
+    t.v.zero_()
+    t.vNew.zero_()
+    j = torch.arange(t.rows, device="cuda")
+    t.v.view(B, t.rows, K, D)[:, j, :, j % D] = 1
+    i = torch.arange(T, device="cuda")
+    for b in range(B):
+        t.vNew.view(B, T, K, D)[b, i, :, (t.lens[b] + i) % D] = 1
+    got = t.call(on_torch, splits=splits).view(B, T, H, D).double()
+    on_torch.sync()
+    half = torch.finfo(t.td).eps / 2
+    for b, L in enumerate(t.lens):
+        seen = torch.tensor(t.seen[b], device="cuda")
+        depth = (seen.sum(-1) - 1).clamp(min=0)
+        past = torch.ones(T, L, dtype=torch.bool, device="cuda")
+        if window is not None:
+            past &= torch.arange(L, device="cuda") >= (L + depth - window)[:, None]
+            seen = seen & (depth[:, None] - depth[None] <= window)
+        mask = torch.cat([past, seen], 1).double()
+        column = torch.nn.functional.one_hot(torch.arange(L + T, device="cuda") % D, D).double()
+        want = (mask @ column / mask.sum(-1, keepdim=True))[:, None]
+        # Weights are powers of two and their sums whole numbers below 2^24: exact, but for the reciprocal and the product with it
+        # (2^-23 each), once for every one of up to 64 parts; and the result's own rounding.  A key more or less is 1/1064.
+        assert ((got[b] - want).abs() <= (half + 66 * 2.0 ** -23) * want + 2.0 ** -25).all(), b
