@@ -513,18 +513,22 @@ RT_API int rt_rotary(rt_ctx* ctx, const rt_rotary_args* args);
  * n_b = nodeCounts[b] drafted tokens (nodes where nodeCounts is NULL), whose keys and values
  * are kNew and vNew and stay outside the cache.  Node i sees the cache rows below L_b and
  * the nodes j < n_b whose bit j of masks[b][i] is set: its ancestors and itself, as a rule.
- * Its depth is the number of other nodes that it sees and its position L_b + depth; with
- * windowLeft it sees no cache row before position - windowLeft and no node whose depth is
- * smaller than its own by more than windowLeft.  Scores, sinks and heads are rt_attn's.  A
+ * Its depth is one less than the number of nodes that it sees (0 if it sees none) and its
+ * position L_b + depth; with windowLeft it sees no cache row before position - windowLeft and
+ * no node whose depth is smaller than its own by more than windowLeft.  Scores, sinks and heads are rt_attn's.  A
  * node that sees nothing, and the nodes past n_b, come out as zeros; caches are only read.
  * kvLen is also the longest L_b to plan for.  An L_b outside [0, cacheRows] or an n_b
  * outside [0, nodes] makes its sequence come out as zeros and rt_sync report it.
  * headDim is at most 128, as in rt_attn_decode.  out overlaps no input.
  *
+ * What a node does not see has no part in its result, whatever it holds; infinities and NaN that
+ * it does see come out as arithmetic has them.
+ *
  * Long caches are cut into parts that meet in the context's scratch: like rt_attn_decode's,
  * calls of one context, and replays of graphs captured from it, follow one another on the
  * GPU.  splits = 1 cuts none and needs no scratch; a first call under a capture, where none
- * can be made, cuts as many as the scratch at hand allows, on the tensor cores none. */
+ * can be made, cuts as many as the scratch at hand allows, on the tensor cores none.  A
+ * captured call keeps the cuts that its kvLen asked for, on every replay. */
 typedef struct {
   const void* q;            /* device [batch*nodes, qHeads*headDim] */
   void* out;                /* device [batch*nodes, qHeads*headDim] */
@@ -550,7 +554,8 @@ typedef struct {
   int32_t headDim;
   int32_t windowLeft;       /* RT_WINDOW_INF = unbounded */
   int32_t sharedMasks;
-  int32_t splits;           /* key splits per sequence; 0 = let the library choose */
+  int32_t splits;           /* key splits per sequence; 0 = let the library choose; on the tensor
+                             * cores more than 1 = cut anywhere, into as many runs as the GPU takes */
 } rt_tree_args;
 RT_API int rt_attn_tree(rt_ctx* ctx, const rt_tree_args* args);
 /* Which kernel rt_attn_tree would run: "tree_tc" (tensor cores) or "tree_simt" (FP32 pipes). */

@@ -984,7 +984,7 @@ int rt_attn_tree(rt_ctx* ctx, const rt_tree_args* a) {
     ctx->launches += launches;
     return RT_OK;
   }
-  rt::plan_tree_simt(p, a->dtype, ctx->smCount);
+  rt::plan_tree_simt(p, ctx->smCount);
   if (p.splits > 1) {
     const size_t perSplit = (size_t)p.batch * p.nodes * p.qHeads * (2 + p.hd) * sizeof(float);
     if (perSplit * p.splits > ctx->scratchBytes && capturing(ctx->stream)) {

@@ -31,7 +31,8 @@ struct TreeParams {
   const int32_t* counts;
   const uint64_t* masks;
   const float* sinks;
-  float* scratch;       // [batch*nodes*qHeads][splits][2+hd] f32 (m, l, acc), used when splits > 1
+  float* scratch;       // FP32 pipes, splits > 1: [batch*nodes*qHeads][splits][2+hd] f32 (m, l, acc); tensor cores, cut inside heads:
+                        // the accumulators, (m, l) and joins of tree_tc.cu's Plan
   int* status;
   int64_t cacheSeqStride, qStride, kNewStride, vNewStride;   // elements
   int32_t batch, nodes, cacheRows, kvLen, qHeads, kvHeads, hd, wl, sharedMasks, splits;
@@ -78,8 +79,8 @@ __device__ __forceinline__ TreeRow tree_row(const TreeParams& p, int b, int i, i
 }
 #endif
 
-// Keys of a tile of the FP32-pipe kernel, and how it cuts the call: fills splits (0 = by the plan).
-void plan_tree_simt(TreeParams& p, int dtype, int smCount);
+// How the FP32-pipe kernel cuts the call: fills splits where they are 0.
+void plan_tree_simt(TreeParams& p, int smCount);
 cudaError_t launch_tree_simt(const TreeParams& p, int dtype, cudaStream_t s);
 // The splits' partials into out, a second launch.
 cudaError_t launch_tree_merge(const TreeParams& p, int dtype, cudaStream_t s);

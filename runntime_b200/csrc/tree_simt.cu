@@ -349,7 +349,7 @@ int rows_of(const TreeParams& p) {
 
 }  // namespace
 
-void plan_tree_simt(TreeParams& p, int, int smCount) {
+void plan_tree_simt(TreeParams& p, int smCount) {
   if (p.splits > 0) return;
   const int bm = rows_of(p), rows = p.nodes * (p.qHeads / p.kvHeads);
   const int64_t units = (int64_t)p.batch * p.kvHeads * ((rows + bm - 1) / bm);

@@ -17,8 +17,8 @@
 // probabilities of one half.)
 //
 // What it takes with 32 heads on 8 of 128: 32 sequences of 8190 rows, 25 tokens 187 us, 4.5 TB/s (the caches' bytes at
-// the copy rate: 128); 16 of 4096 at most, 16 tokens 55.5 us, 3.7 TB/s, of which some 9 pass before the first product and 6 in
-// the joining launch; one of 65001, 64 tokens 111 us, 614 TFLOP/s counting each product once: a chain of scores, softmax and the
+// the copy rate: 128); 16 of 4096 at most, 16 tokens 56 us, 3.7 TB/s, of which some 9 pass before the first product and 6 in
+// the joining launch; one of 65001, 64 tokens 110 us, 619 TFLOP/s counting each product once: a chain of scores, softmax and the
 // product of the probabilities, whose place the next scores take.  (Probabilities of one half, 11 bits: 162, 53 and 92 us.)
 // The smallest, 8 heads of 52, 190 rows and 7 tokens: 12 us, all of it latency.
 //

@@ -239,7 +239,8 @@ def tree_batched(ex: CudaExecutor, q, out, kCache, vCache, kNew, vNew, masks, *,
     include/rt_attn.h.  ``q``/``out``: [batch*nodes, qHeads*headDim]; ``kNew``/``vNew``: the tokens' own keys and
     values, which stay outside the caches; ``masks``: device int64 [batch, nodes] (or [nodes] with
     ``sharedMasks``), see tree_masks.  ``kvLens`` (device int32 [batch]) are the rows in the caches, ``kvLen`` their
-    maximum, or the length of all without them; ``nodeCounts`` the sequences' own numbers of nodes."""
+    maximum, or the length of all without them; ``nodeCounts`` the sequences' own numbers of nodes.  A captured call
+    keeps the plan for its ``kvLen``."""
     # (fields in the order of the structure)
     call(ex._lib, "rt_attn_tree", ex.ctx, TreeArgs, q, out, kCache, vCache, kNew, vNew, kvLens, nodeCounts, masks, sinks,
          cacheRows * kvHeads * headDim if cacheSeqStride is None else cacheSeqStride, qRowStride, kNewRowStride,
@@ -429,7 +430,9 @@ class KvCacheEngine:
     def stepTree(self, q, kNew, vNew, out, masks, *, nodes: int, nodeCounts=None, sharedMasks: bool = False,
                  qRowStride: int = 0, kNewRowStride: int = 0, vNewRowStride: int = 0, sinks=None) -> None:
         """``nodes`` drafted tokens of every sequence attend to its cache and to their ancestors
-        (tree_batched).  Nothing is appended: commitTree does that for the tokens that stand."""
+        (tree_batched).  Nothing is appended: commitTree does that for the tokens that stand.  A captured step keeps the
+        plan of the lengths at its capture: replayed with caches many times as long it is right, but slower than a step captured at
+        such lengths (or a tree_batched with kvLen = cacheRows)."""
         device = self.lens.device
         _check_tensor("stepTree", "masks", masks, "int64", device, 1 if sharedMasks else self.batch, nodes, nodes)
         _check_tensor("stepTree", "nodeCounts", nodeCounts, "int32", device, 1, self.batch, self.batch)
