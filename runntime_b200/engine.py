@@ -308,12 +308,13 @@ def _each(tensors):
 
 def _check_tensor(call: str, name: str, x, kind: str, device, rows: int, cols: int, stride: int) -> None:
     """Refuses a tensor that does not hold what a kernel reads from its address on: ``rows`` times ``cols`` numbers
-    of ``kind``, ``stride`` elements from one row to the next.  Addresses are taken as they are."""
+    of ``kind`` (or, of integers, the unsigned kind), ``stride`` elements from one row to the next.  Addresses are
+    taken as they are."""
     if not hasattr(x, "dtype"):
         return
     if x.device != device:
         raise ValueError(f"{call}: {name} is on {x.device}, not on {device}")
-    if str(x.dtype) != "torch." + kind:
+    if str(x.dtype) not in ("torch." + kind, "torch.u" + kind):
         raise ValueError(f"{call}: {name} is {x.dtype}, not torch.{kind}")
     if x.is_contiguous() and (x.dim() != 2 or rows == 1 or x.shape[1] == stride):
         fits = cols == 0 or x.numel() >= (rows - 1) * stride + cols

@@ -139,6 +139,7 @@ def test_masks_counts_and_sinks_that_a_step_takes_and_refuses(monkeypatch):
     i32, f32 = torch.int32, torch.float32
     call(z(3, 5))
     call(z(15))
+    call(z(3, 5).view(torch.uint64))
     call(z(5), sharedMasks=True)
     call(z(3, 5), sharedMasks=True)
     call(z(5, 5)[1:4], nodeCounts=z(3, dtype=i32), sinks=z(4, dtype=f32))
